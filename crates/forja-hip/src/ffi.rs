@@ -160,6 +160,7 @@ extern "C" {
     pub fn fh_write(backend: *mut fh_backend, buffer: fh_buffer, byte_offset: u64, bytes: *const c_void, len: u64) -> u32;
     pub fn fh_read(backend: *mut fh_backend, buffer: fh_buffer, byte_offset: u64, bytes: *mut c_void, len: u64) -> u32;
     pub fn fh_read_tensor(backend: *mut fh_backend, tensor: *const fh_tensor, bytes: *mut c_void, len: u64) -> u32;
+    pub fn fh_device_address(backend: *mut fh_backend, buffer: fh_buffer, address: *mut u64) -> u32;
     pub fn fh_prepare_program(
         backend: *mut fh_backend,
         kind: u32,

@@ -2874,6 +2874,15 @@ fh_status fh_read_tensor(fh_backend *b, const fh_tensor *tensor, void *bytes, ui
   return FH_OK;
 }
 
+fh_status fh_device_address(fh_backend *b, fh_buffer buffer, uint64_t *address) {
+  if (!b || !address) return FH_INVALID_INPUT;
+  std::lock_guard<std::mutex> lock(b->mutex);
+  const auto it = b->allocations.find(buffer);
+  if (it == b->allocations.end()) return FH_INVALID_INPUT;
+  *address = (uint64_t)(uintptr_t)it->second.ptr;
+  return FH_OK;
+}
+
 fh_status fh_prepare_program(fh_backend *b, uint32_t kind, const fh_inst *insts, uint32_t n_insts,
                              const uint32_t *outputs, uint32_t n_pairs, fh_program *out) {
   if (!b || !insts || !outputs || !out) return FH_INVALID_INPUT;

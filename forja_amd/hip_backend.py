@@ -63,7 +63,7 @@ class FhDeviceInfo(C.Structure):
 
 EXPORTS = [
     "fh_create", "fh_destroy", "fh_alloc", "fh_release", "fh_import", "fh_write", "fh_read",
-    "fh_read_tensor", "fh_prepare_program", "fh_release_program", "fh_submit", "fh_submit_static", "fh_wait",
+    "fh_read_tensor", "fh_device_address", "fh_prepare_program", "fh_release_program", "fh_submit", "fh_submit_static", "fh_wait",
     "fh_gpu_time_ns", "fh_submission_free", "fh_device_info_get", "fh_memory_usage", "fh_set_memory_limit",
     "fh_submit_profiled", "fh_submission_profile",
     "fh_synchronize", "fh_profile_enable", "fh_profile_select", "fh_profile_sample", "fh_profile_reset", "fh_profile_read",
@@ -92,6 +92,7 @@ def load_library():
     lib.fh_write.argtypes = [vp, u64, u64, vp, u64]
     lib.fh_read.argtypes = [vp, u64, u64, vp, u64]
     lib.fh_read_tensor.argtypes = [vp, C.POINTER(FhTensor), vp, u64]
+    lib.fh_device_address.argtypes = [vp, u64, C.POINTER(u64)]
     lib.fh_prepare_program.argtypes = [vp, u32, C.POINTER(FhInst), u32, C.POINTER(u32), u32,
                                        C.POINTER(u64)]
     lib.fh_release_program.argtypes = [vp, u64]
@@ -263,6 +264,12 @@ class HipBackend:
         out = (C.c_char * max(end - start, 1))()
         _check(self._lib.fh_read(self._handle, buffer, start, out, end - start))
         return bytes(out[:end - start])
+
+    def device_address(self, tensor: Tensor) -> int:
+        """Where the tensor's first element lies on the device (fh_device_address: order and lifetime)."""
+        address = C.c_uint64()
+        _check(self._lib.fh_device_address(self._handle, tensor.buffer, C.byref(address)))
+        return address.value + tensor.layout.offset * tensor.layout.dtype.byte_size
 
     def release(self, tensor: Tensor) -> None:
         _check(self._lib.fh_release(self._handle, tensor.buffer))

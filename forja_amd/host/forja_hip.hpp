@@ -401,6 +401,13 @@ class HipBackend {
     r.error.code = fh_read(raw_, buffer, byte_offset, r.value.data(), len);
     return r;
   }
+  // Where the tensor's first element lies on the device (fh_device_address).
+  Result<uint64_t> device_address(const Tensor &tensor) {
+    Result<uint64_t> r;
+    r.error.code = fh_device_address(raw_, tensor.buffer, &r.value);
+    if (r.ok()) r.value += tensor.layout.offset * dtype_bytes(tensor.dtype);
+    return r;
+  }
   Result<Unit> release(const Tensor &tensor) {
     Result<Unit> r;
     r.error.code = fh_release(raw_, tensor.buffer);

@@ -221,6 +221,11 @@ FH_API fh_status fh_read(fh_backend *backend, fh_buffer buffer, uint64_t byte_of
                   uint64_t len);
 /* Backend::read (lib.rs:141-148): gathers a strided view into logical row-major bytes. */
 FH_API fh_status fh_read_tensor(fh_backend *backend, const fh_tensor *tensor, void *bytes, uint64_t len);
+/* Where an allocation lies on the device, until it is released: for a caller whose own kernels, or another
+ * library's, read results or write inputs in place (no counterpart in the reference).  Work on the device's
+ * null stream comes after what was submitted before it and before what is submitted after it; other streams
+ * are the caller's to order.  Weights are written by fh_write: the library keeps operands made from them. */
+FH_API fh_status fh_device_address(fh_backend *backend, fh_buffer buffer, uint64_t *address);
 /* Backend::prepare_program (lib.rs:1357-1363) / prepare_epilogue: validates and stores the IR. */
 FH_API fh_status fh_prepare_program(fh_backend *backend, uint32_t kind /* 0 map, 1 row */,
                              const fh_inst *insts, uint32_t n_insts,
