@@ -215,69 +215,89 @@ def _the_backend():
     return _backend
 
 
+class _Buffer:
+    """A tensor of the framework and the memory under it, as torch takes it; released with the last tensor over it."""
+
+    def __init__(self, backend, dtype, shape):
+        self.backend, self.tensor = backend, backend.alloc(dtype, tuple(shape))
+        bytes_ = self.tensor.layout.buffer_len
+        self.__cuda_array_interface__ = {"shape": (bytes_,), "typestr": "|u1", "strides": None, "version": 2,
+                                         "data": (backend.device_address(self.tensor), False)}
+
+    def __del__(self):
+        if self.backend._handle is not None:
+            self.backend.release(self.tensor)
+
+
 class _Device:
-    """The state on the device, as the framework's tensors, and the recorded command list."""
+    """The state in the framework's tensors, and the recorded command list.  torch's own stream here is the null stream, which
+    comes after what the backend has been given, and before what it is given next."""
 
     def __init__(self, case, s):
         from forja_amd.core import INTO_PAGES, OUT_OF_PAGES, CommandList, DType, Op
-        self.backend, self.tensors = _the_backend(), []
+        self.backend, self.buffers, self.kind = _the_backend(), [], s.kind
         dtype = {"bf16": DType.BF16, "f16": DType.F16, "f32": DType.F32}[case["dtype"]]
-        total, pt, heads, dim = s.codes[0].shape
-        u32 = lambda t: self._put(DType.U32, t.shape, t.cpu().numpy().astype(np.uint32))  # noqa: E731
-        words = lambda t: self._put(DType.U32, (*t.shape[:-1], t.shape[-1] // 4), t.cpu().numpy())  # noqa: E731
-        floats = lambda t: self._put(dtype, t.shape, (t if t.dtype == torch.float32 else t.view(torch.int16)).cpu().numpy())  # noqa: E731
-        self.codes, self.scales = [words(t) for t in s.codes], words(s.scales)
+        planes, (total, pt, heads, dim) = len(s.codes), s.codes[0].shape
+        u32 = lambda t: self._put(DType.U32, t.shape, t.to(torch.int32))[0]  # noqa: E731
+        words = lambda t: self._put(DType.U32, (*t.shape[:-1], t.shape[-1] // 4), t)  # noqa: E731
+        floats = lambda t: self._put(dtype, t.shape, t)  # noqa: E731
+        pools, codes = words(torch.cat(s.codes))
+        pools = [pools.narrow(0, plane * total, total) for plane in range(planes)]
+        all_scales, scales = words(s.scales)
+        # where the pass's rows lie, [plane, row, head]: the row's codes, and its scale
+        plane = torch.arange(planes, device="cuda")[:, None]
+        self.codes, self.scales = codes.view(-1, heads, dim), scales.view(-1)
+        self.rows = ((plane * total + s.page) * pt + s.slot).flatten()
+        self.places = ((((s.page * planes + plane) * heads)[..., None] + torch.arange(heads, device="cuda")) * pt + s.slot[:, None]).flatten()
+        self.shape = planes, len(s.page), heads, dim
         generations = u32(s.generations)
         commands = CommandList()
         if s.kind == "attend":
             tables, cu, starts = u32(s.tables), u32(torch.from_numpy(s.cu)), u32(s.starts)
-            self.out = floats(s.out)
+            out, self.out = floats(s.out)
             commands.dispatch_many(
                 Op.paged_quant_attention_ragged(s.scale, pt, one_row_per_lane=case["rows"] == 0),
-                [floats(s.q), *(floats(t) for t in s.new), tables, generations, cu, starts],
-                [self.out, *self.codes, self.scales])
+                [floats(s.q)[0], *(floats(t)[0] for t in s.new), tables, generations, cu, starts], [out, *pools, all_scales])
         else:
-            table = u32(s.tables[0])
-            scales = self.scales.reshape((total, heads, pt // 4))
+            table, plane_scales = u32(s.tables[0]), all_scales.reshape((total, heads, pt // 4))
             if s.kind == "write":
                 commands.dispatch_many(Op.paged_quant_copy(INTO_PAGES, case["start"], pt),
-                                       [floats(s.new[0]), table, generations], [self.codes[0], scales])
+                                       [floats(s.new[0])[0], table, generations], [pools[0], plane_scales])
+                out, self.out = self._put(DType.F32, self.shape[1:], torch.zeros(self.shape[1:], device="cuda"))
             else:
-                self.out = floats(s.out)
-                commands.dispatch_many(Op.paged_quant_copy(OUT_OF_PAGES, case["start"], pt),
-                                       [self.codes[0], scales, table, generations], [self.out])
+                out, self.out = floats(s.out)
+            commands.dispatch_many(Op.paged_quant_copy(OUT_OF_PAGES, case["start"], pt),
+                                   [pools[0], plane_scales, table, generations], [out])
         self.encoded = self.backend.encode(commands)
 
-    def _put(self, dtype, shape, array):
-        tensor = self.backend.alloc(dtype, tuple(shape))
-        self.tensors.append(tensor)
-        if array.any():
-            self.backend.write_array(tensor, array)
-        return tensor
+    def _put(self, dtype, shape, values):
+        """The framework's tensor of `values`, and torch's over the same memory."""
+        buffer = _Buffer(self.backend, dtype, shape)
+        self.buffers.append(buffer)
+        held = torch.as_tensor(buffer, device="cuda").view(values.dtype).view(values.shape)
+        held.copy_(values)
+        return buffer.tensor, held
 
-    def __del__(self):
-        if self.backend._handle is not None:
-            for tensor in self.tensors:
-                self.backend.release(tensor)
-
-    def submit(self):
+    def run(self):
+        """One pass, and its outputs whole: the output rows where the framework has put them, and what the rows that it has
+        stored stand for (of one sequence, as it reads them back)."""
         _submitted.append(self.backend.submit(self.encoded))
         if len(_submitted) > IN_FLIGHT:
             _submitted.popleft().wait()
-
-    def read(self, tensor, dtype):
-        while _submitted:
-            _submitted.popleft().wait()
-        return torch.frombuffer(bytearray(self.backend.read_buffer_range(tensor.buffer, 0, tensor.layout.buffer_len)), dtype=dtype)
+        if self.kind == "read":
+            return {"out": self.out}
+        exponents = self.scales.index_select(0, self.places).int()
+        if self.kind == "write":
+            return {"rows": self.out, "exponents": exponents.sub_(127).view(self.shape[1:3])}
+        rows = self.codes.index_select(0, self.rows).view(torch.float8_e4m3fn).float().view(self.shape)
+        rows *= (exponents << 23).view(torch.float32).view(*self.shape[:3], 1)
+        return {"out": self.out, "keys": rows[0], "values": rows[1]}
 
 
 def prepare(case, seed):
     s = _inputs(case, seed)
     if own:
         s.device = _Device(case, s)
-        s.host = {name: t.cpu() for name, t in (("page", s.page), ("slot", s.slot))}
-        s.shapes = [t.shape for t in s.codes], s.scales.shape, getattr(s, "out", torch.zeros(0)).shape
-        s.dtype = TORCH[case["dtype"]]
         for name in ("codes", "scales", "new", "q", "out", "tables", "generations"):
             s.__dict__.pop(name, None)
     return s
@@ -354,7 +374,7 @@ def _attend_lanes(s, lanes, row0, rows):
 def run(state):
     s = state
     if own:
-        s.device.submit()
+        return s.device.run()
     elif s.kind == "read":
         s.out.copy_(_decoded(s.codes[0][s.page, s.slot], s.scales[s.page, 0, :, s.slot].int() - 127))
     else:
