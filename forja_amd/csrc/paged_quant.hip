@@ -887,6 +887,14 @@ struct Queries {
   uint32_t exponent;   // the byte of 2^e
 };
 
+// The byte of a row's 2^e.  The second e4m3 pieces count 2^(e - 4), whose byte has to be one too: 5 at least (rows below 2^-113;
+// their elements then lie lower in the codes' range, and the smallest come to 2^-135, far below what their scores tell apart).
+template <bool kWide>
+__device__ inline uint32_t query_scale_byte(float most) {
+  const uint32_t byte = scale_byte(most);
+  return kWide ? byte : max(byte, 5u);
+}
+
 // Sixteen query elements as pieces; `inverse`: 2^-e.  (No number stays one: its code, or f16's.)
 template <bool kWide>
 __device__ inline void query_pieces(const float (&x)[16], float inverse, uint32_t *first, uint32_t *second) {
@@ -947,7 +955,7 @@ __device__ inline void make_queries(const QuantBatch &p, Queries<D, kWide> &q, c
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[j][i] = 0.0f;
   }
-  q.exponent = scale_byte(max_of_quarters(largest_query(x)));
+  q.exponent = query_scale_byte<kWide>(max_of_quarters(largest_query(x)));
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) query_pieces<kWide>(x[j], inverse_scale_of(q.exponent), q.piece[0][j], q.piece[1][j]);
 }
@@ -1489,7 +1497,7 @@ __device__ inline void make_prompt_queries(const QuantBatch &p, PromptQueries<D,
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[j][i] *= sign;
-  q.exponent = scale_byte(max_of_halves(largest_query(x)));
+  q.exponent = query_scale_byte<kWide>(max_of_halves(largest_query(x)));
 #pragma unroll
   for (int j = 0; j < D / 32; ++j)
     query_pieces<kWide>(x[j], inverse_scale_of(q.exponent), q.piece[0][j / 2] + (kWide ? 8 : 4) * (j % 2),

@@ -611,3 +611,20 @@ def test_two_backends_at_once():
         want, bound = batch.expected(0.09)
         within(got, want, bound)
         backend.close()
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 30, 3]])
+@pytest.mark.parametrize("width", [64, 128])
+def test_queries_of_any_size(hip, counts, width):
+    """Rows down to the smallest numbers of bf16, whose elements do not come down to one code each: every key then weighs alike,
+    and a row is nearly the mean of its values.  And rows of 2^100 under a scale that takes them back."""
+    for dtype, out_dtype in ((DType.BF16, DType.BF16), (DType.BF16, DType.F16), (DType.F32, DType.F32)):
+        batch = Batch([70, 5, 600], counts, 8, 2, 16, width, dtype=dtype, out_dtype=out_dtype, seed=71)
+        sizes = np.arange(-133, -109)
+        sizes = np.resize(sizes, batch.q.shape[:2])[..., None]       # every size, with each element's own bits
+        batch.q = rounded(np.ldexp(batch.q / np.abs(batch.q).max(-1, keepdims=True), sizes), dtype)
+        got = batch.check(hip, 1.0)
+        assert np.abs(got).max() > 0
+        batch = Batch([70, 5, 600], counts, 8, 2, 16, width, dtype=dtype, out_dtype=out_dtype, seed=72)
+        batch.q = rounded(batch.q * 2.0 ** 100, dtype)
+        batch.check(hip, 0.09 * 2.0 ** -100)
