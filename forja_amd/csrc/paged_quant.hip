@@ -637,9 +637,9 @@ __device__ inline void make_plan(const QuantBatch &p, PlanShared<kThreads> &s, E
   __syncthreads();
   const uint32_t units = s.units;
   const uint64_t most_keys = min((uint64_t)p.table_pages * p.page_tokens, (uint64_t)0xffffffffu);
-  // A unit's lane, first token, tokens, and keys of its last one; 0 keys: they pass the lane's table.
+  // A unit's lane, first token, tokens, and keys of the last of them (0: none); and the tokens behind them that pass the lane's table.
   struct Unit {
-    uint32_t lane, token, members, keys;
+    uint32_t lane, token, members, keys, past;
     bool prompt;   // of a lane that brings several tokens
   };
   auto unit_at = [&](uint32_t unit) {
@@ -648,9 +648,11 @@ __device__ inline void make_plan(const QuantBatch &p, PlanShared<kThreads> &s, E
     const uint32_t n = s.lane_cu[u.lane + 1] - s.lane_cu[u.lane], each = unit_tokens(n), index = (unit - s.unit_first[u.lane]) * each;
     u.prompt = p.prompt_tokens != 0 && n > 1;
     u.token = s.lane_cu[u.lane] + index;
-    u.members = min(each, n - index);
-    const uint64_t keys = (uint64_t)s.lane_start[u.lane] + index + u.members;
-    u.keys = keys > most_keys ? 0u : (uint32_t)keys;
+    const uint32_t all = min(each, n - index);
+    const uint64_t before = (uint64_t)s.lane_start[u.lane] + index;
+    u.members = before < most_keys ? (uint32_t)min((uint64_t)all, most_keys - before) : 0u;
+    u.past = all - u.members;
+    u.keys = u.members ? (uint32_t)before + u.members : 0u;
     return u;
   };
   {
@@ -736,21 +738,22 @@ __device__ inline void make_plan(const QuantBatch &p, PlanShared<kThreads> &s, E
   const uint32_t each = p.prompt_tokens != 0 || 8 * units <= kThreads ? 8 : 1, part = thread % each;
   for (uint32_t unit = thread / each; unit < units; unit += kThreads / each) {
     const Unit u = unit_at(unit);
-    uint32_t chunk = 0, splits = 0, listed = 0;
+    uint32_t chunk = 0, splits = 1, listed = 0;
     if (u.keys != 0) {
       const uint32_t of = split_of(u, &chunk, &splits);
       if (part == 0) atomicAdd(&s.class_items[of], splits);
-    } else if (part == 0) {
-      report_error(error, p.table_pages);
     }
     if (part == 0 && splits != 1) listed = atomicAdd(splits > kFewSplits ? &s.merge_count : &s.few_count, u.members);
     listed = __shfl(listed, (int)(lane_id - part), 64);
     const uint32_t base = base_of(u);
     for (uint32_t m = part; m < u.members; m += each) {
-      const uint64_t keys = (uint64_t)s.lane_start[u.lane] + (u.token - s.lane_cu[u.lane]) + m + 1;
       p.bad[u.token + m] = 0;
-      p.tokens_of[u.token + m] = make_uint2(u.lane, keys > most_keys ? 0u : (uint32_t)keys);
+      p.tokens_of[u.token + m] = make_uint2(u.lane, u.keys - u.members + m + 1);
       if (splits != 1) p.merge[splits > kFewSplits ? listed + m : p.tokens - 1 - listed - m] = make_uint4(u.token + m, splits, base + m * p.prompt_splits, 0);
+    }
+    if (part == 0 && u.past != 0) {
+      report_error(error, p.table_pages);
+      zero_rows(u.token + u.members, u.token + u.members + u.past);
     }
   }
   __syncthreads();
@@ -1656,7 +1659,9 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
   const uint32_t longest = item.attended + item.members - 1;
   const uint32_t begin = item.split * item.chunk, end = min(longest, begin + item.chunk);
   const uint32_t *table = p.tables + (uint64_t)item.lane * p.table_pages * 2;
-  const uint32_t first_page = begin / pt, last_page = (end - 1) / pt;
+  const uint32_t first_page = begin / pt;
+  uint32_t last_page = (end - 1) / pt;
+  uint32_t refused_from = 0xffffffffu;   // the first key of the first page that is refused: rows that attend it are zeros
   // What does not wait for anything is requested first: up to 64 table entries at once (by every wave for itself: same
   // entries, same result), and the queries.
   auto request_entry = [&](uint32_t page0) {
@@ -1698,20 +1703,20 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
     const uint32_t my_page = page0 + lane, physical = entry.x;
     const bool mine = my_page <= last_page, ok = !mine || (physical < p.physical_pages && p.generations[physical] == entry.y);
     const unsigned long long bad_mask = __ballot(!ok);
-    if (bad_mask) {
-      if (wave == 0 && lane == (uint32_t)__ffsll((long long)bad_mask) - 1) {
-        report_error(error, my_page);
-        for (uint32_t m = 0; m < item.members; ++m) p.bad[item.leader + m] = 1;
-      }
-      if (item.splits == 1 && used) {   // no merge follows
-        const uint64_t to = (uint64_t)(item.leader + member) * p.out_stride_t + (uint64_t)head * p.out_stride_h;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) store_out4(p, to + D / 2 * half + 4 * c, 0.f, 0.f, 0.f, 0.f);
-      }
-      return;
-    }
     const uint32_t low = max(begin, page0 * pt);
-    const uint32_t high = (uint32_t)min((uint64_t)end, ((uint64_t)page0 + 64) * pt);
+    uint32_t high = (uint32_t)min((uint64_t)end, ((uint64_t)page0 + 64) * pt);
+    if (bad_mask) {
+      const uint32_t refused = page0 + (uint32_t)__ffsll((long long)bad_mask) - 1;
+      refused_from = refused * pt;
+      if (wave == 0 && my_page == refused) {
+        report_error(error, refused);
+        for (uint32_t m = refused_from >= item.attended ? refused_from - item.attended + 1 : 0; m < item.members; ++m) p.bad[item.leader + m] = 1;
+      }
+      if (refused_from <= low) break;
+      last_page = refused - 1;
+      high = refused_from;
+      wave_end = min(wave_end, refused_from);
+    }
     const uint32_t limit = min(own_limit, high), group_end = min(wave_end, high);
     const uint32_t start = min(low + 16 * wave, (high - 1) & ~15u);
     StageCursor at{start / pt - page0, start % pt};
@@ -1745,6 +1750,7 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
     __syncthreads();   // the next tile staged goes into the first buffer
   }
   if (clean_from != 0xffffffffu) {
+    wave_end = min(wave_end, refused_from);
     const uint32_t first_token = p.cu[item.lane], row_bytes = p.kv_heads * D;
     for (uint32_t base = max(begin, new_from); base < wave_end; base += 64) {
       const uint32_t mine = base + lane;
@@ -1767,7 +1773,7 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
   sm.l += __shfl_xor(sm.l, 32, 64);
   if (!used) return;
   // This lane holds value columns 32c + 8n + 4 * half + 0..3 of its row in o[c][4n..4n + 3].
-  const bool single = item.splits == 1;
+  const bool single = item.splits == 1, zero = single && item.attended + member > refused_from;   // (of several splits the merge knows)
   const float inverse = single ? 1.0f / sm.l : 1.0f;
   const uint64_t slot = (uint64_t)(item.base + member * p.prompt_splits + item.split) * p.query_heads + head;
   const uint64_t to = (uint64_t)(item.leader + member) * p.out_stride_t + (uint64_t)head * p.out_stride_h;
@@ -1778,7 +1784,7 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
       const uint32_t column = 32 * c + 8 * n + 4 * half;
       const float x = o[c][4 * n] * inverse, y = o[c][4 * n + 1] * inverse, z = o[c][4 * n + 2] * inverse, w = o[c][4 * n + 3] * inverse;
       if (single)
-        store_out4(p, to + column, x, y, z, w);
+        store_out4(p, to + column, zero ? 0.0f : x, zero ? 0.0f : y, zero ? 0.0f : z, zero ? 0.0f : w);
       else
         *(float4 *)(p.partial_o + slot * D + column) = make_float4(x, y, z, w);
     }

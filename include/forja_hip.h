@@ -131,7 +131,9 @@ typedef enum fh_op_kind {
   FH_OP_PAGED_QUANT_COPY = 35,
   /* FH_OP_PAGED_ATTENTION_RAGGED over an 8-bit cache: each lane's new K/V rows are stored at its q_start as
    * FH_OP_PAGED_QUANT_COPY stores them, then attended with the rest as the cache holds them.  Inputs, `k`,
-   * the precondition and what is refused on the device as there.  `bits` = 8.
+   * the precondition and what is refused on the device as there.  `bits` = 8.  A new row whose page entry is
+   * not authentic is not stored, a row that attends a page whose entry is not reads zero, and so does one that
+   * passes its lane's table; the lowest such logical page is reported, and the lane's other rows are attended.
    *   outputs: out [T,Hq,Dv] float, key codes u32 [P,pt,Hkv,D/4], value codes u32 [P,pt,Hkv,Dv/4],
    *            scales u32 [P,2,Hkv,ceil(pt/4)] (plane 0 keys, 1 values)
    * D <= 512, Dv <= 256.  With f32 outputs, or queries of f32 or f16, scores and weights carry at least 16

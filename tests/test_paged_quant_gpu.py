@@ -628,3 +628,48 @@ def test_queries_of_any_size(hip, counts, width):
         batch = Batch([70, 5, 600], counts, 8, 2, 16, width, dtype=dtype, out_dtype=out_dtype, seed=72)
         batch.q = rounded(batch.q * 2.0 ** 100, dtype)
         batch.check(hip, 0.09 * 2.0 ** -100)
+
+
+@pytest.mark.parametrize("hq,hkv,pt,width", [(8, 4, 16, 128), (20, 4, 16, 128), (16, 1, 64, 64), (8, 4, 16, 96), (9, 3, 48, 128)])
+@pytest.mark.parametrize("context,count,first", [(70, 30, 80), (0, 200, 96), (3000, 160, 3072), (3000, 160, 2496), (40, 9, 48)])
+@pytest.mark.parametrize("past", [False, True])
+def test_rows_before_a_refused_page_are_attended(hip, hq, hkv, pt, width, context, count, first, past):
+    """A chunk of which a page is stale, or whose rows pass the lane's table, from about position `first` on: rows that attend
+    nothing of it are as without it, those that do are zeros, and what has a page of its own is stored."""
+    page = -(-first // pt)
+    position = context + np.arange(count)
+    lost = position[position >= page * pt if past else position // pt == page]
+    reached = np.zeros(count + 4, bool)
+    reached[1:1 + count] = position + 1 > page * pt
+    # (strange: values of no number among the new rows)
+    for dtype, strange in ((DType.BF16, False), (DType.BF16, True), (DType.F32, True)):
+        batch, whole = (Batch([33, context, 5], [1, count, 3], hq, hkv, pt, width, dtype=dtype, seed=81) for _ in range(2))
+        for b in (batch, whole):
+            if strange:
+                b.v_new[1 + count // 3, 0, 5] = b.v_new[count, hkv - 1, 0] = np.nan
+        if past and reached.any():
+            batch.tables = batch.tables[:, :page]
+        else:
+            batch.tables[1, page, 1] ^= 1
+        batch.upload(hip)
+        if reached.any():
+            with pytest.raises(BackendError) as info:
+                batch.attend(hip, 0.09)
+            assert info.value.status == Status.DEVICE_ERROR_FLAG and info.value.index == page
+        else:
+            batch.attend(hip, 0.09)
+        got = to_f32(hip.read(batch.out), dtype).reshape(*batch.q.shape[:2], -1)
+        want, bound = whole.expected(0.09)
+        assert not got[reached].any()
+        got, want, bound = got[~reached], want[~reached], bound[~reached]
+        number = ~np.isnan(want)
+        assert np.array_equal(np.isnan(got), ~number)
+        within(got[number], want[number], bound[number])
+        at, slot = whole.where(1, lost)
+        for held, first_held in zip(whole.codes, batch.codes):
+            held[at, slot] = first_held[at, slot]
+        whole.scales[at, :, :, slot] = batch.scales[at, :, :, slot]
+        for tensor, array in zip(batch.cache, (*whole.codes, whole.scales)):
+            got = read_bytes(hip, tensor).reshape(array.shape)
+            none = (array & 0x7f) == 0x7f                   # the sign of no number is not told
+            assert np.array_equal(got & 0x7f, array & 0x7f) and np.array_equal(got[~none], array[~none])
