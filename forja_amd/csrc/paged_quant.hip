@@ -468,6 +468,7 @@ struct QuantBatch {
   // Tokens of a unit of a lane that brings several; 0: every token is a unit of its own (a decode batch).
   uint32_t prompt_tokens;
   uint32_t max_splits, prompt_splits;   // most splits of a unit of one token and of others
+  uint32_t single_slots;                // partial slots of units of one token, in front of those of others
   uint32_t item_slots;                  // workgroups that the device holds at once, over those of an item of one token
   uint32_t promised, append_in_kernel;
   uint32_t not_finite;                  // what counts[4] holds if a new value row is not finite, and not_finite_rows of its token
@@ -732,7 +733,7 @@ __device__ inline void make_plan(const QuantBatch &p, PlanShared<kThreads> &s, E
     return (u.prompt ? 64 : 0) + min(*chunk / kTile, 63u);
   };
   auto base_of = [&](const Unit &u) {
-    return u.prompt ? p.lanes * p.max_splits + u.token * p.prompt_splits : (p.prompt_tokens ? u.lane : u.token) * p.max_splits;
+    return u.prompt ? p.single_slots + u.token * p.prompt_splits : (p.prompt_tokens ? u.lane : u.token) * p.max_splits;
   };
   // Eight threads a unit, for its tokens and splits; one where the units are many and each is a token.
   const uint32_t each = p.prompt_tokens != 0 || 8 * units <= kThreads ? 8 : 1, part = thread % each;
@@ -2022,14 +2023,17 @@ bool run_fast(fh_backend *backend, const RaggedQuantAttention &p, ErrorSlot *err
   static uint32_t known[2][2][2][9];   // [width][wide][prompts][waves]
   const uint32_t held = resident(kernel, 64 * waves, &known[p.width / 128][wide][prompts][waves]);
   f.item_slots = std::max(held * backend_compute_units(backend) / per_item, 1u);
-  // Partial slots: of the tokens, or of the lanes that bring one and of the tokens of others.
+  // Partial slots: of the tokens, or of the lanes that bring one and of the tokens of others; none of a unit that is not split.
   const uint32_t singles = prompts ? f.lanes : f.tokens;
   f.max_splits = std::max(1u, std::min(kMostSplits, (prompts ? 8192u : 16384u) / singles));
   f.prompt_splits = prompts ? std::max(1u, std::min(64u, 8192u / f.tokens)) : 0;
   const uint64_t row_bytes = (uint64_t)f.query_heads * p.width * sizeof(float);
-  auto slots = [&] { return (uint64_t)singles * f.max_splits + (uint64_t)f.tokens * f.prompt_splits; };
+  auto slots = [&] {
+    f.single_slots = f.max_splits > 1 ? singles * f.max_splits : 0;
+    return f.single_slots + (f.prompt_splits > 1 ? (uint64_t)f.tokens * f.prompt_splits : 0);
+  };
   auto ml_bytes = [&] { return round_256(slots() * f.query_heads * sizeof(float2)); };
-  auto partial_bytes = [&] { return ml_bytes() + slots() * row_bytes; };
+  auto partial_bytes = [&] { return ml_bytes() + slots() * row_bytes + 256; };   // (never nothing: a null workspace is a refused one)
   while (partial_bytes() > backend_workspace_limit(backend) && (f.max_splits > 1 || f.prompt_splits > 1)) {
     if (f.max_splits >= f.prompt_splits)
       --f.max_splits;

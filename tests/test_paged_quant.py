@@ -153,3 +153,27 @@ refused(op, ins(), outs()[:3])
 pool = codes()
 refused(op, ins(), outs(kc=pool, vc=pool))
 """)
+
+
+def test_workspace_is_asked_for_the_splits_there_are(fake):  # noqa: F811
+    """Rows that are attended in one piece have no partial results: static submissions take any number of them, and ordinary ones
+    keep no memory for them."""
+    fake("""
+def batch(tokens, lanes, heads, promise=False):
+    pools = [hip.alloc(DType.U32, (4, 16, 4, 32)) for _ in range(2)] + [hip.alloc(DType.U32, (4, 2, 4, 4))]
+    rows = [hip.alloc(DType.BF16, (tokens, h, 128)) for h in (heads, 4, 4)]
+    words = [hip.alloc(DType.U32, s) for s in ((lanes, 4, 2), (4,), (lanes + 1,), (lanes,))]
+    commands = CommandList()
+    commands.dispatch_many(Op.paged_quant_attention_ragged(0.1, 16, promise), rows + words, [hip.alloc(DType.BF16, (tokens, heads, 128)), *pools])
+    return commands
+for tokens, lanes, heads in ((2600, 1, 32), (9000, 3, 32), (2600, 2600, 32), (700, 2, 128)):
+    for promise in {False, tokens == lanes}:
+        launched()
+        hip.submit_static(batch(tokens, lanes, heads, promise))
+        assert any("prompt_kernel" in name or "decode_kernel" in name for name in launched())
+big = batch(8256, 70, 40)
+held = hip.memory_usage()
+hip.submit(big).wait()
+# 117 splits of 70 lanes' single rows; 20 KiB and 8 bytes a head for each
+assert hip.memory_usage() - held < (70 * 117 * 40 * 520 + (4 << 20)), hip.memory_usage() - held
+""")

@@ -673,3 +673,10 @@ def test_rows_before_a_refused_page_are_attended(hip, hq, hkv, pt, width, contex
             got = read_bytes(hip, tensor).reshape(array.shape)
             none = (array & 0x7f) == 0x7f                   # the sign of no number is not told
             assert np.array_equal(got & 0x7f, array & 0x7f) and np.array_equal(got[~none], array[~none])
+
+
+@pytest.mark.parametrize("contexts,counts", [([0, 300, 20], [600, 1, 40]), ([(37 * i) % 50 for i in range(650)], [1] * 650)])
+def test_static_batches_whose_splits_do_not_fit(hip, contexts, counts):
+    """A partial row for every token of these batches is more than a static submission's 36 MiB: they are attended unsplit."""
+    assert sum(counts) * 128 * 128 * 4 > 36 << 20
+    Batch(contexts, counts, 128, 8, 16, seed=91).check(hip, 0.09, static=True)
