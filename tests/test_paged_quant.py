@@ -177,3 +177,29 @@ hip.submit(big).wait()
 # 117 splits of 70 lanes' single rows; 20 KiB and 8 bytes a head for each
 assert hip.memory_usage() - held < (70 * 117 * 40 * 520 + (4 << 20)), hip.memory_usage() - held
 """)
+
+
+@pytest.mark.parametrize("promise", [False, True])
+def test_a_plan_ends_with_the_lanes_that_it_is_of(fake, promise):  # noqa: F811
+    """Layers of a submission share a plan until one of its inputs is written; static submissions too."""
+    fake(CACHE + f"""
+tokens, promise = {3 if promise else 9}, {promise}
+op = Op.paged_quant_attention_ragged(0.1, pt, promise)
+rows = [hip.alloc(DType.BF16, (tokens, h, D)) for h in (4, H, H)]
+words = [tables, gens, cu, starts, active]
+out, pools = hip.alloc(DType.BF16, (tokens, 4, D)), [codes(), codes(), scales()]
+for written in words + [pools[2]]:
+    source = hip.alloc(DType.U32, written.shape)
+    commands = CommandList()
+    for layer in range(2):
+        commands.dispatch_many(op, rows + words, [out, *pools])
+    commands.dispatch(Op.copy(), [source], written)
+    for layer in range(2):
+        commands.dispatch_many(op, rows + words, [out, *pools])
+    for submit_list in (lambda: hip.submit(commands).wait(), lambda: hip.submit_static(commands)):
+        launched()
+        submit_list()
+        names = ["plan" if "prepare_kernel" in n else "attend" for n in launched() if "prepare_kernel" in n or "prompt_kernel" in n or "decode_kernel" in n]
+        want = ["plan", "attend", "attend"] * 2 if written is not pools[2] else ["plan"] + ["attend"] * 4
+        assert names == want, (written.shape, names)
+""")

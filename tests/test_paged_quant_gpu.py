@@ -680,3 +680,36 @@ def test_static_batches_whose_splits_do_not_fit(hip, contexts, counts):
     """A partial row for every token of these batches is more than a static submission's 36 MiB: they are attended unsplit."""
     assert sum(counts) * 128 * 128 * 4 > 36 << 20
     Batch(contexts, counts, 128, 8, 16, seed=91).check(hip, 0.09, static=True)
+
+
+@pytest.mark.parametrize("static", [False, True])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 30, 3]])
+def test_lanes_that_change_between_layers(hip, counts, static):
+    """A list that writes the lanes' starts and tables between two layers: each is attended, and stored, by its own."""
+    first, later = (Batch(contexts, counts, 16, 8, 16, seed=seed) for contexts, seed in (([70, 300, 5], 31), ([9, 2, 64], 34)))
+    pages = max(b.tables.shape[1] for b in (first, later))
+    physical = max(b.physical for b in (first, later))
+    for batch in (first, later):
+        empty = np.tile(np.array([0, 0xffffffff], np.uint32), (3, pages - batch.tables.shape[1], 1))
+        batch.tables = np.concatenate([batch.tables, empty], 1)
+        more = physical - batch.physical
+        batch.codes = [np.concatenate([c, np.full((more, *c.shape[1:]), 0x7f, np.uint8)]) for c in batch.codes]
+        batch.scales = np.concatenate([batch.scales, np.full((more, *batch.scales.shape[1:]), 247, np.uint8)])
+        batch.physical = physical
+        batch.upload(hip)
+    commands = CommandList()
+    op = Op.paged_quant_attention_ragged(0.09, 16, max(counts) == 1)
+    held = first.inputs[3:]                                   # what both layers name
+    commands.dispatch_many(op, first.inputs, [first.out, *first.cache])
+    for index in (3, 6):
+        commands.dispatch(Op.copy(), [later.inputs[index]], held[index - 3])
+    commands.dispatch_many(op, later.inputs[:3] + held, [later.out, *later.cache])
+    if static:
+        hip.submit_static(commands)
+    else:
+        hip.submit(commands).wait()
+    for batch in (first, later):
+        want, bound = batch.expected(0.09)
+        within(to_f32(hip.read(batch.out), DType.BF16).reshape(want.shape), want, bound)
+        for tensor, array in zip(batch.cache, (*batch.codes, batch.scales)):
+            assert np.array_equal(read_bytes(hip, tensor).reshape(array.shape), array)
