@@ -1949,17 +1949,20 @@ BatchKernel prompt_kernel(uint32_t width, bool wide) {
   return wide ? quant_prompt_kernel<128, true> : quant_prompt_kernel<128, false>;
 }
 
-// Workgroups of `kernel` that a compute unit holds; asked once a kernel (every writer stores the same value).
-uint32_t resident(BatchKernel kernel, uint32_t threads, uint32_t *known) {
-  if (*known == 0) {
+// Workgroups of `kernel` that a compute unit holds; asked once a kernel, by whichever backend's thread comes first (others
+// that ask meanwhile store the same value).
+uint32_t resident(BatchKernel kernel, uint32_t threads, std::atomic<uint32_t> *known) {
+  uint32_t held = known->load(std::memory_order_relaxed);
+  if (held == 0) {
     int blocks = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, (int)threads, 0) != hipSuccess || blocks < 1) {
       (void)hipGetLastError();
       blocks = 1;
     }
-    *known = (uint32_t)blocks;
+    held = (uint32_t)blocks;
+    known->store(held, std::memory_order_relaxed);
   }
-  return *known;
+  return held;
 }
 
 bool fast_eligible(const RaggedQuantAttention &p) {
@@ -2020,7 +2023,7 @@ bool run_fast(fh_backend *backend, const RaggedQuantAttention &p, ErrorSlot *err
   const uint32_t places = f.kv_heads * f.head_tiles, waves = prompts ? kPromptWaves : std::min(places, 8u);
   const uint32_t per_item = (places + waves - 1) / waves;
   BatchKernel kernel = prompts ? prompt_kernel(p.width, wide) : decode_kernel(p.width, wide);
-  static uint32_t known[2][2][2][9];   // [width][wide][prompts][waves]
+  static std::atomic<uint32_t> known[2][2][2][9];   // [width][wide][prompts][waves]
   const uint32_t held = resident(kernel, 64 * waves, &known[p.width / 128][wide][prompts][waves]);
   f.item_slots = std::max(held * backend_compute_units(backend) / per_item, 1u);
   // Partial slots: of the tokens, or of the lanes that bring one and of the tokens of others; none of a unit that is not split.
