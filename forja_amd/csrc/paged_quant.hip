@@ -882,8 +882,10 @@ __device__ inline void query_values(const QuantBatch &p, const RawQuery<kWide> &
 
 // The queries of a wave's 16 rows (this lane: 16 elements of each 64, of row `lane & 15`) as operands of the matrix cores.
 //   kWide false: e4m3 pieces x = 2^e (c_0 + c_1 / 16) for the scaled products with the codes as they are.  Two hold the 8
-//     bits of a bf16 element down to 2^-11 of the row's largest, and what is smaller to 2^-22 of it.  (These products keep
-//     about 2^-13 of their largest term: below what bf16 weights round.)
+//     bits of a bf16 element down to 2^-11 of the row's largest, and what is smaller to 2^-22 of it.  (These products sum terms
+//     of any size to 2^-14 of the largest, root mean square, at worst to 2^-11 of it or 2^-12 of the sum of all sizes; a large
+//     term beside small ones to 2^-16, at worst 2^-12.7; operands within a factor of nine exactly.  For scores of a few units
+//     that is below what bf16 weights round.)
 //   kWide true: f16 pieces x = 2^e (h_0 + h_1 / 2^11), 22 bits, for products with the codes as f16.
 template <int D, bool kWide>
 struct Queries {

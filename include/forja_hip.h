@@ -138,7 +138,7 @@ typedef enum fh_op_kind {
    *            scales u32 [P,2,Hkv,ceil(pt/4)] (plane 0 keys, 1 values)
    * D <= 512, Dv <= 256.  With f32 outputs, or queries of f32 or f16, scores and weights carry at least 16
    * bits; with bf16 queries and 16-bit outputs the softmax weights are rounded to bf16, and the products of a
-   * score are summed to about 2^-13 of the largest of them. */
+   * score are summed to about 2^-14 of the largest of them, at worst 2^-11. */
   FH_OP_PAGED_QUANT_ATTENTION_RAGGED = 36
 } fh_op_kind;
 

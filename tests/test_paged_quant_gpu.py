@@ -713,3 +713,35 @@ def test_lanes_that_change_between_layers(hip, counts, static):
         within(to_f32(hip.read(batch.out), DType.BF16).reshape(want.shape), want, bound)
         for tensor, array in zip(batch.cache, (*batch.codes, batch.scales)):
             assert np.array_equal(read_bytes(hip, tensor).reshape(array.shape), array)
+
+
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 40, 3]])
+def test_one_channel_that_dominates_the_scores(hip, width, counts):
+    """Keys and queries with one channel hundreds of times as large as the others', which almost every key has alike: what tells
+    keys apart is the rest.  A product of two codes is exact; summed by a scaled product of the matrix cores, terms end
+    2^-11.9 of the sum of all sizes from the exact sum at worst (measured: 64 and 128 terms of sizes spread over 2^34, and one large one
+    beside small ones, 2^-12 and 2^-12.7); the second pieces add terms of at most 2^-4 of the first ones' sizes, so that a score of bf16
+    queries may be off by 2^-11.5 S where the other forms' are by 2^-14 S (see the head of this file)."""
+    scale = 0.02
+
+    def rows(rng):
+        def make(what, shape):
+            values = rng.standard_normal(shape) * 0.3
+            if what != "v":
+                values[..., 7] = 20.0 + rng.integers(-1, 2, shape[:-1])
+            return values
+        return make
+
+    for dtype, sums in ((DType.BF16, 2.0 ** -11.5), (DType.F32, 0.0)):
+        batch = Batch([70, 300, 600], counts, 8, 2, 16, width, dtype=dtype, make=rows(np.random.default_rng(101)), seed=101)
+        got = batch.upload(hip).attend(hip, scale)
+        want, bound = batch.expected(scale)
+        for lane, (context, count) in enumerate(zip(batch.contexts, counts)):
+            page, slot = batch.where(lane, np.arange(context + count))
+            keys, values = (quant_cache.decode_rows(batch.codes[p][page, slot], batch.scales[page, p, :, slot]) for p in range(2))
+            at = slice(batch.cu[lane], batch.cu[lane + 1])
+            o, a, s = quant_cache.attend(batch.q[at].astype(np.float64), keys, values, float(np.float32(scale)), context + 1 + np.arange(count))
+            assert s.min() > 6
+            bound[at] += 2 * sums * s * a
+        within(got, want, bound)
