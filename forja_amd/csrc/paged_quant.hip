@@ -1111,8 +1111,9 @@ __device__ inline void consume_tile(const QuantTile<D> &cur, const Queries<D, kW
     sm.m = m_new;
   }
   sm.l += sum;
-  // The weights: one bf16 each (8 bits, as the output of that form), or three that hold all their 24 bits.
-  constexpr int kPieces = kWide ? 3 : 1;
+  // The weights: two bf16 each (16 bits; with one the errors of bf16 rows against 64 bits are 0.0019 instead of 0.0017, most of it
+  // the output's rounding, and no batch is faster), or three that hold all their 24 bits.
+  constexpr int kPieces = kWide ? 3 : 2;
   uint32_t pieces[kPieces][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -1519,8 +1520,9 @@ __device__ inline f32x16 mfma_bf16(const uint4 &a, const uint4 &b, const f32x16 
 // `masked` false: every key of the tile is below every limit.  scale_log2 is positive.
 //
 // The sums follow every new maximum, so that the weight of the largest score is exactly 1 (with sums that follow only what is
-// 2^8 times larger: 2048 rows 94 us instead of 99, errors against 64 bits 2.3e-3 instead of 2.0e-3); bf16 weights are summed
-// as they are rounded.
+// 2^8 times larger: 2048 rows 94 us instead of 99, errors against 64 bits 2.3e-3 instead of 2.0e-3).  bf16 rows weigh with one
+// bf16, summed as it is rounded (with two, errors are 1.7e-3, most of it the output's own rounding, but the products are what bounds this kernel:
+// 2048 rows and 32 lanes 111 -> 129 us in all, 8256 rows 250 -> 293).
 template <int D, bool kWide>
 __device__ inline void attend_tile(const QuantBatch &p, const TilePlaces<D, kWide> &at, uint32_t buffer, const PromptQueries<D, kWide> &q,
                                    f32x16 (&o)[D / 32], Softmax &sm, bool masked, uint32_t tile0, uint32_t limit, float scale_log2,

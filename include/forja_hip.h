@@ -136,9 +136,9 @@ typedef enum fh_op_kind {
    * passes its lane's table; the lowest such logical page is reported, and the lane's other rows are attended.
    *   outputs: out [T,Hq,Dv] float, key codes u32 [P,pt,Hkv,D/4], value codes u32 [P,pt,Hkv,Dv/4],
    *            scales u32 [P,2,Hkv,ceil(pt/4)] (plane 0 keys, 1 values)
-   * D <= 512, Dv <= 256.  With f32 outputs, or queries of f32 or f16, scores and weights carry at least 16
-   * bits; with bf16 queries and 16-bit outputs the softmax weights are rounded to bf16, and the products of a
-   * score are summed to about 2^-14 of the largest of them, at worst 2^-11. */
+   * D <= 512, Dv <= 256.  Softmax weights carry at least 16 bits, and so do scores with f32 outputs, or queries
+   * of f32 or f16.  With bf16 queries and 16-bit outputs the products of a score are summed to about 2^-14 of the
+   * largest of them, at worst 2^-11, and the weights of a lane that brings several rows are rounded to bf16. */
   FH_OP_PAGED_QUANT_ATTENTION_RAGGED = 36
 } fh_op_kind;
 

@@ -745,3 +745,20 @@ def test_one_channel_that_dominates_the_scores(hip, width, counts):
             assert s.min() > 6
             bound[at] += 2 * sums * s * a
         within(got, want, bound)
+
+
+@pytest.mark.parametrize("width", [64, 128])
+def test_decode_weights_hold_16_bits(hip, width):
+    """Rows of bf16 with few keys, to f16: the bound of a decode batch with weights of 2^-16, and scores as the scaled products sum
+    them (2^-11.5 S: see the test of a dominating channel; S is small here)."""
+    batch = Batch([i % 7 for i in range(200)], [1] * 200, 8, 2, 16, width, out_dtype=DType.F16, seed=111)
+    got = batch.upload(hip).attend(hip, 0.004)
+    want, bound = batch.expected(0.004)
+    for lane, context in enumerate(batch.contexts):
+        page, slot = batch.where(lane, np.arange(context + 1))
+        keys, values = (quant_cache.decode_rows(batch.codes[p][page, slot], batch.scales[page, p, :, slot]) for p in range(2))
+        o, a, s = quant_cache.attend(batch.q[lane:lane + 1].astype(np.float64), keys, values, float(np.float32(0.004)), [context + 1])
+        assert s.max() < 1
+        bound[lane] = (HALF_STEP[DType.F16] * np.abs(o) + (2.0 ** -16 + 2 * (2.0 ** -11.5 * s + 2.0 ** -18 * s + 2.0 ** -21)
+                                                         + (context / 4 + 64) * 2.0 ** -23) * a + 2.0 ** -25)[0]   # (f16's smallest step)
+    within(got, want, bound)
