@@ -762,3 +762,18 @@ def test_decode_weights_hold_16_bits(hip, width):
         bound[lane] = (HALF_STEP[DType.F16] * np.abs(o) + (2.0 ** -16 + 2 * (2.0 ** -11.5 * s + 2.0 ** -18 * s + 2.0 ** -21)
                                                          + (context / 4 + 64) * 2.0 ** -23) * a + 2.0 ** -25)[0]   # (f16's smallest step)
     within(got, want, bound)
+
+
+@pytest.mark.parametrize("counts,activity,lead,behind", [([1, 700, 3, 40], [1, 0, 1, 1], 0, 900), ([1, 5, 1, 2], [1, 1, 0, 1], 70, 1200),
+                                                         ([1, 1, 1, 1], [1, 1, 1, 0], 0, 300), ([600, 1, 300, 1], [0, 0, 0, 0], 5, 0)])
+def test_padded_batches(hip, counts, activity, lead, behind):
+    """Rows in front of the first lane, behind the last and of inactive lanes, more of them than the plan has threads: all read zero."""
+    batch = Batch([40, 0, 700, 3], counts, 8, 2, 16, activity=activity, seed=121)
+    shift = lambda a: np.concatenate([np.ones((lead, *a.shape[1:]), np.float32), a, np.ones((behind, *a.shape[1:]), np.float32)])  # noqa: E731
+    batch.q, batch.k_new, batch.v_new = (shift(a) for a in (batch.q, batch.k_new, batch.v_new))
+    batch.cu = batch.cu + lead
+    got = batch.check(hip, 0.09)
+    live = np.zeros(len(got), bool)
+    for lane, active in enumerate(activity):
+        live[batch.cu[lane]:batch.cu[lane + 1]] = active
+    assert not got[~live].any() and got[live].any(axis=(1, 2)).all()
