@@ -244,6 +244,7 @@ class _Device:
         pools, codes = words(torch.cat(s.codes))
         pools = [pools.narrow(0, plane * total, total) for plane in range(planes)]
         all_scales, scales = words(s.scales)
+        plane_scales = [all_scales.reshape((total, planes * heads, pt // 4)).narrow(1, plane * heads, heads) for plane in range(planes)]
         # where the pass's rows lie, [plane, row, head]: the row's codes, and its scale
         plane = torch.arange(planes, device="cuda")[:, None]
         self.codes, self.scales = codes.view(-1, heads, dim), scales.view(-1)
@@ -258,16 +259,26 @@ class _Device:
             commands.dispatch_many(
                 Op.paged_quant_attention_ragged(s.scale, pt, one_row_per_lane=case["rows"] == 0),
                 [floats(s.q)[0], *(floats(t)[0] for t in s.new), tables, generations, cu, starts], [out, *pools, all_scales])
+            # what the stored rows stand for: of few sequences as the framework reads them back, a dispatch a sequence and plane
+            self.read_back = len(s.counts) <= 8
+            if self.read_back:
+                rows, self.stored = self._put(DType.F32, self.shape, torch.zeros(self.shape, device="cuda"))
+                for plane in range(planes):
+                    for lane, (context, count) in enumerate(zip(s.contexts, s.counts)):
+                        commands.dispatch_many(
+                            Op.paged_quant_copy(OUT_OF_PAGES, context, pt),
+                            [pools[plane], plane_scales[plane], tables.narrow(0, lane, 1).reshape(tables.shape[1:]), generations],
+                            [rows.narrow(0, plane, 1).reshape(self.shape[1:]).narrow(0, int(s.cu[lane]), count)])
         else:
-            table, plane_scales = u32(s.tables[0]), all_scales.reshape((total, heads, pt // 4))
+            table = u32(s.tables[0])
             if s.kind == "write":
                 commands.dispatch_many(Op.paged_quant_copy(INTO_PAGES, case["start"], pt),
-                                       [floats(s.new[0])[0], table, generations], [pools[0], plane_scales])
+                                       [floats(s.new[0])[0], table, generations], [pools[0], plane_scales[0]])
                 out, self.out = self._put(DType.F32, self.shape[1:], torch.zeros(self.shape[1:], device="cuda"))
             else:
                 out, self.out = floats(s.out)
             commands.dispatch_many(Op.paged_quant_copy(OUT_OF_PAGES, case["start"], pt),
-                                   [pools[0], plane_scales, table, generations], [out])
+                                   [pools[0], plane_scales[0], table, generations], [out])
         self.encoded = self.backend.encode(commands)
 
     def _put(self, dtype, shape, values):
@@ -280,12 +291,14 @@ class _Device:
 
     def run(self):
         """One pass, and its outputs whole: the output rows where the framework has put them, and what the rows that it has
-        stored stand for (of one sequence, as it reads them back)."""
+        stored stand for."""
         _submitted.append(self.backend.submit(self.encoded))
         if len(_submitted) > IN_FLIGHT:
             _submitted.popleft().wait()
         if self.kind == "read":
             return {"out": self.out}
+        if self.kind == "attend" and self.read_back:
+            return {"out": self.out, "keys": self.stored[0], "values": self.stored[1]}
         exponents = self.scales.index_select(0, self.places).int()
         if self.kind == "write":
             return {"rows": self.out, "exponents": exponents.sub_(127).view(self.shape[1:3])}
