@@ -195,8 +195,9 @@ __global__ __launch_bounds__(256) void quant_store_kernel(QuantCopy p, ErrorSlot
             (uint8_t *)p.scales.base + 4 * (p.scales.offset + page * p.scales.stride[0] + head * p.scale_words) + slot);
 }
 
-// The same in pieces.  What bounds it: HBM; of few rows the chain table, generation, store.  (32749 rows of 8 heads of 128, 101 MB:
-// 26 us, 3.9 TB/s; by the kernel above 105.)
+// The same in pieces.  What bounds it: the vector ALUs, which find row, head, page and slot for every eight values (177 instructions a
+// wave, busy 0.75 of the time), next to HBM; of few rows the chain table, generation, store.  (32749 rows of 8 heads of 128, 101 MB:
+// 27 us, 3.7 TB/s; by the kernel above 105.)
 template <uint32_t kLanes>
 __global__ __launch_bounds__(256) void quant_store_rows_kernel(QuantCopy p, ErrorSlot *error) {
   const uint32_t flat = blockIdx.x * 256 + threadIdx.x, row = flat / kLanes, piece = flat % kLanes;
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(256) void quant_store_rows_kernel(QuantCopy p, Erro
                       (uint8_t *)p.scales.base + 4 * (p.scales.offset + page * p.scales.stride[0] + head * p.scale_words) + slot);
 }
 
-// Eight codes a thread out of the pages: HBM (16384 rows of 4 heads of 128 to f32, 42 MB: 13 us, 3.2 TB/s; the kernel below 18).
+// Eight codes a thread out of the pages.  What bounds it: the chain table, generation, codes, store of every wave (waiting 0.61 of its
+// time), two rounds of workgroups of it for 16384 rows of 4 heads of 128 to f32 (42 MB: 13.5 us, 3.1 TB/s; the kernel below 18).
 __global__ __launch_bounds__(256) void quant_load_rows_kernel(QuantCopy p, ErrorSlot *error) {
   const uint32_t flat = blockIdx.x * 256 + threadIdx.x, pieces = p.words / 2;
   if (flat >= p.tokens * p.heads * pieces || !quant_active(p.activity)) return;
@@ -1315,8 +1317,8 @@ __device__ inline void attend_token(const QuantBatch &p, ErrorSlot *error, const
 }
 
 // A workgroup is one item; its waves take one kv head (and 16 of its query heads) each, so that the rows of all heads of
-// a token are requested close together in time.  What bounds it: HBM (128 lanes of 256 to 32768 keys, 888 MB: 153 us, 5.8 TB/s);
-// of few keys the chain item, table entry and generation, codes, and the launch (400 keys 7.7 us).  In between the start of
+// a token are requested close together in time.  What bounds it: HBM (128 lanes of 256 to 32768 keys, 888 MB: 156 us, 5.7 TB/s);
+// of few keys the chain item, table entry and generation, codes, and the launch (400 keys 8.0 us).  In between the start of
 // every item, next to four to eight tiles of it (48 lanes of 128 to 4096 keys, 115 MB: 26 us; 8 f32 lanes of up to 32768, 55 MB: 20).
 template <int D, bool kWide>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void quant_decode_kernel(QuantBatch p, ErrorSlot *error) {
@@ -1344,7 +1346,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // The 16-byte piece p of a key's row r sits in slot p ^ (r & 7) (64 values: p ^ (r >> 1 & 3)): eight rows read at one piece
 // use all banks once.  Piece p of a value's row r sits in slot p ^ ((r & 3) << 2 | (r >> 2 & 3)) (64 values: p ^
 // ((r >> 1 & 1) << 2 | (r >> 2 & 3))): the transposing read takes 4 rows x 4 pieces at once, which the first term spreads
-// over the banks.  Keys past the end of a split are taken from a valid row and masked; values past it are zeros.
+// over the banks.  (Conflicts are counted all the same: 3.6e7 cycles for 2048 rows behind 16384 keys, about a tenth of the time of 256
+// compute units; which of the accesses make them is not known.)  Keys past the end of a split are taken from a valid row and
+// masked; values past it are zeros.
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
@@ -1809,9 +1813,10 @@ __device__ inline void attend_unit(const QuantBatch &p, ErrorSlot *error, uint32
 // A batch with prompt rows: the items of several tokens, the kv heads of an item side by side (with 8, 4, 2 or 1 kv heads
 // a head's items then meet in the L2 of one XCD, as workgroups go to the XCDs in turn), and behind them those of one token,
 // four waves of a kv head each.  What bounds it: instructions of both kinds, one wave's matrix products hardly running beside
-// the other's softmax (matrix cores busy 49 %, vector ALUs 53 % of the time; raising a wave's priority over one or the other
-// part changes nothing): 2048 rows behind 16384 keys, 32 heads, 665 us, 0.88 PFLOP/s; 8192 rows of 6 prompts and 64 lanes,
-// 40 heads, 235 us, 0.57, where a unit's start (list, entries, first tile: 6 us) is as long as three tiles.  f32: 3 us a tile.
+// the other's softmax (matrix cores busy 49 %, vector ALUs 52 % of the time; raising a wave's priority over one or the other
+// part changes nothing): 2048 rows behind 16384 keys, 32 heads, 629 us, 0.93 PFLOP/s; 8192 rows of 6 prompts and 64 lanes,
+// 40 heads, 235 us, 0.57, where a unit's start (list, entries, first tile: 6 us) is as long as three tiles.  f32: 3 us a tile; heads of
+// 128 then need more registers than there are (30 spilled, 116 bytes of scratch a lane, most of them around a unit's start and end).
 template <int D, bool kWide>
 __global__ __launch_bounds__(64 * kPromptWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void quant_prompt_kernel(QuantBatch p, ErrorSlot *error) {
   __shared__ uint4 tiles[2 * Staged<D>::kBytes / 16];
