@@ -631,7 +631,7 @@ def test_queries_of_any_size(hip, counts, width):
 
 
 @pytest.mark.parametrize("hq,hkv,pt,width", [(8, 4, 16, 128), (20, 4, 16, 128), (16, 1, 64, 64), (8, 4, 16, 96), (9, 3, 48, 128)])
-@pytest.mark.parametrize("context,count,first", [(70, 30, 80), (0, 200, 96), (3000, 160, 3072), (3000, 160, 2496), (40, 9, 48)])
+@pytest.mark.parametrize("context,count,first", [(70, 30, 80), (0, 200, 96), (3000, 160, 3088), (3000, 160, 2496), (40, 9, 48)])
 @pytest.mark.parametrize("past", [False, True])
 def test_rows_before_a_refused_page_are_attended(hip, hq, hkv, pt, width, context, count, first, past):
     """A chunk of which a page is stale, or whose rows pass the lane's table, from about position `first` on: rows that attend
